@@ -72,10 +72,11 @@ __global__ void __launch_bounds__(256) step_maps_kernel(const StepMapsParams p) 
     const bool bad = p.q_lens[b] < 0 || p.kv_before[b] < 0 || need_l > p.max_blocks || ids + need_l > p.num_ids ||
                      rows + q > p.T;
     if (lane0 == 0) {
+      // what does not fit stays inside the step's rows: whoever indexes by these may rely on it
       if (bad) status_set(kStatusBadIndex);
-      p.q_starts[b] = static_cast<int>(rows);
-      p.kv_lens[b] = kv + q;
-      p.logit_rows[b] = static_cast<int>(rows) + q - 1;
+      p.q_starts[b] = static_cast<int>(min(rows, static_cast<long>(p.T)));
+      p.kv_lens[b] = static_cast<int>(min(static_cast<long>(kv) + q, 0x7fffffffl));
+      p.logit_rows[b] = static_cast<int>(min(rows + q, static_cast<long>(p.T))) - 1;
     }
     const int need = static_cast<int>(min(min(need_l, static_cast<long>(p.max_blocks)), max(0l, p.num_ids - ids)));
     const int* mine = p.blocks + ids;
@@ -86,9 +87,14 @@ __global__ void __launch_bounds__(256) step_maps_kernel(const StepMapsParams p) 
     for (int i = lane0; i < q; i += step) {
       const long t = rows + i;
       if (t >= p.T) break;
-      const int key = kv + i, blk = key / p.page;
-      p.slots[t] = blk < need ? mine[blk] * p.page + key % p.page : -1;
-      int pos = key;
+      // unsigned, and slots in 64 bits: a length near 2^31 must not become a key in front of the table, nor a block id
+      // that is none the slot of another one
+      const uint32_t key = static_cast<uint32_t>(kv) + i, page = p.page, blk = key / page;
+      const bool held = blk < static_cast<uint32_t>(need);
+      const long slot = held ? static_cast<long>(mine[blk]) * p.page + key % page : -1;
+      if (held && (slot < 0 || slot > 0x7fffffffl)) status_set(kStatusBadIndex);
+      p.slots[t] = slot < 0 || slot > 0x7fffffffl ? -1 : static_cast<int>(slot);
+      int pos = static_cast<int>(key);
       if (p.depths) {
         const int node = tree - q + i;
         const bool inside = node >= 0 && node < p.depth_nodes;
