@@ -197,7 +197,19 @@ class LLMEngine:
         with N.device_of(self.device):
             masks, depths = TR.tree_plan(links)
         self.spec_tree = branching
-        self._tree = dict(levels=levels, parents=links, masks=masks, depths=depths, nodes=len(parents))
+        paths = [(n, a) for n in range(1, len(parents)) for a in self._ancestors(parents, n)]
+        rows, nodes = torch.tensor(paths, dtype=torch.int32, device=self.device).t().contiguous()
+        self._tree = dict(levels=levels, parents=links, masks=masks, depths=depths, nodes=len(parents), path_rows=rows,
+                          path_nodes=nodes)
+
+    @staticmethod
+    def _ancestors(parents: Sequence[int], n: int) -> List[int]:
+        """Node n and the nodes on its way to the root, without the root (the last accepted token)."""
+        out = []
+        while n > 0:
+            out.append(n)
+            n = parents[n]
+        return out
 
     def add_request(self, prompt: Sequence[int], params: SamplingParams, soft: Optional[dict] = None) -> int:
         """``soft`` describes a multimodal prompt: ``rows`` (prompt positions of the placeholder tokens), ``vals``
@@ -354,7 +366,9 @@ class LLMEngine:
             batch.bidir = (i32([u[0] for u in runs]), i32([u[1] for u in runs]), i32([u[2] for u in runs]),
                            batch.block_tables.index_select(0, which).contiguous(), max(u[1] for u in runs), row_idx)
 
-    def _pick_tokens(self, logits: torch.Tensor, reqs: List[Request]) -> torch.Tensor:
+    def _pick_tokens(self, logits: torch.Tensor, reqs: List[Request], drafted: Optional[tuple] = None) -> torch.Tensor:
+        """A token per row of logits, with the row's request's sampler.  ``drafted`` = (tokens, rows): drafted tokens in
+        front of a row that its request has not accepted yet, which a penalty counts for that row."""
         if any(r.params.grammar is not None for r in reqs):
             # Grammar-constrained rows: every token the grammar cannot continue with goes to -inf.  The masks are
             # computed on the host (C++ recogniser stepped over the vocabulary) and applied on the device.
@@ -375,6 +389,8 @@ class LLMEngine:
         if any(r.params.needs_penalties for r in reqs):
             rows = torch.tensor([max(r.row, 0) for r in reqs], device=dev)
             cnt = self.counts.index_select(0, rows) if self.counts is not None else None
+            if drafted is not None:
+                S.count_tokens(cnt, *drafted)
             f = lambda key: torch.tensor([getattr(r.params, key) for r in reqs], dtype=torch.float32, device=dev)
             lg = S.penalties(logits, cnt, f("repetition_penalty"), f("frequency_penalty"), f("presence_penalty"))
         else:
@@ -739,7 +755,10 @@ class LLMEngine:
         if all(r.params.greedy and not r.params.needs_penalties for r in reqs):
             target = self.model.greedy_tokens(logits)
         else:
-            target = self._pick_tokens(logits, [r for r in reqs for _ in range(nodes)])
+            # behind a node come the drafts on its way from the root: a penalty counts them, as it would have by then
+            row, node = t["path_rows"], t["path_nodes"]
+            seen = tokens.index_select(1, node).view(-1), (ar[:, None] * nodes + row).view(-1)
+            target = self._pick_tokens(logits, [r for r in reqs for _ in range(nodes)], seen)
         caches = [(self.cache.k, self.cache.v, slots)]
         if separate:
             held = torch.full((B, nodes), -1, dtype=torch.int32, device=dev)

@@ -100,6 +100,21 @@ def test_sampled_requests_run_over_trees():
     assert all(len(r.token_ids) == 6 and all(0 <= t < 512 for t in r.token_ids) for r in out)
 
 
+@pytest.mark.parametrize("penalty", [dict(repetition_penalty=1.2), dict(frequency_penalty=0.5), dict(presence_penalty=0.7)])
+@pytest.mark.parametrize("tree", [(2, 2, 2), (3, 1, 1, 1)])
+def test_penalties_count_the_drafts_in_front_of_a_node(penalty, tree):
+    """A twin of the target drafts long accepted paths; the token behind each of their nodes is penalised for the drafts on
+    the way, so that the output is that of the engine without a draft."""
+    sp = SamplingParams(max_tokens=14, **penalty)
+    plain = [r.token_ids for r in _engine().generate(PROMPTS, sp)]
+    for kw in (dict(draft_model=_model()), dict(draft_layers=1)):
+        eng = _engine(spec_tree=tree, **kw)
+        assert [r.token_ids for r in eng.generate(PROMPTS, sp)] == plain
+    mixed = [sp, SamplingParams(max_tokens=14), sp]               # requests of both kinds in a round
+    plain = [r.token_ids for r in _engine().generate(PROMPTS, mixed)]
+    assert [r.token_ids for r in _engine(spec_tree=tree, draft_model=_model()).generate(PROMPTS, mixed)] == plain
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="needs a draft"):
         _engine(spec_tree=(2,))
