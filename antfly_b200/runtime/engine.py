@@ -652,7 +652,9 @@ class LLMEngine:
             target = self.model.greedy_tokens(logits)
         else:
             rep = [r for r in reqs for _ in range(K + 1)]
-            target = self._pick_tokens(logits, rep)
+            row, at = torch.tril_indices(K + 1, K, -1, dtype=torch.int32, device=self.device)   # row j: drafts 0 .. j - 1
+            seen = draft.index_select(1, at).int().view(-1), (ar[:, None] * (K + 1) + row).view(-1)
+            target = self._pick_tokens(logits, rep, seen)
         n_m, nxt = S.spec_verify(draft, target.view(B, K + 1).contiguous())
         res = torch.stack([n_m, nxt], 1).cpu().tolist()
         dr = draft.cpu().tolist()

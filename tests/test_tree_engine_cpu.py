@@ -115,6 +115,14 @@ def test_penalties_count_the_drafts_in_front_of_a_node(penalty, tree):
     assert [r.token_ids for r in _engine(spec_tree=tree, draft_model=_model()).generate(PROMPTS, mixed)] == plain
 
 
+@pytest.mark.parametrize("penalty", [dict(repetition_penalty=1.2), dict(frequency_penalty=0.5)])
+def test_penalties_count_the_drafts_in_front_of_a_chains_row(penalty):
+    sp = SamplingParams(max_tokens=14, **penalty)
+    plain = [r.token_ids for r in _engine().generate(PROMPTS, sp)]
+    for kw in (dict(draft_model=_model()), dict(draft_layers=1)):
+        assert [r.token_ids for r in _engine(spec_k=3, **kw).generate(PROMPTS, sp)] == plain
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="needs a draft"):
         _engine(spec_tree=(2,))
