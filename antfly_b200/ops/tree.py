@@ -35,6 +35,7 @@ from . import reference as R
 from .kv_quant import CodecLayer
 
 MAX_NODES = 256       # nodes of one tree
+MIN_SCALE, MAX_SCALE = 1e-7, 1e4     # of the scores of tree attention
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 
@@ -176,7 +177,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     of the tree and the nodes whose bit is set in its own mask row: ``masks`` [B, nodes, ceil(nodes / 32)] from
     :func:`tree_plan`, or any other; a batch dimension expanded from 1 serves one tree shape for all.  A row that sees
     no key comes back as zeros.  ``window`` > 0 (needs ``depths``) keeps the keys at positions > the row's position -
-    ``window``, a node's position being the tree's first key plus its depth.
+    ``window``, a node's position being the tree's first key plus its depth.  ``scale`` (default 1 / sqrt(D)) is a positive
+    number from 1e-7 to 1e4.
 
     ``max_q_len`` bounds ``q_lens`` and ``max_kv`` (0: what the block table can hold) bounds ``kv_lens``; both size the
     launch.  Rows of ``out`` that belong to no sequence are left as they were; in a new output those behind the last
@@ -213,6 +215,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     if out is not None and (out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device):
         raise ValueError(f"out must be bf16 {list(q.shape)} on {q.device}")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if not MIN_SCALE <= scale <= MAX_SCALE:
+        raise ValueError(f"scale must be a positive number from {MIN_SCALE:g} to {MAX_SCALE:g}, got {scale}")
     if not q.is_cuda:
         y = R.tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens, masks, tree_lens, scale, window,
                              depths, out)

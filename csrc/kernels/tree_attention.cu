@@ -1458,6 +1458,12 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
                    B, Hq, Hkv, D, num_blocks, page, nodes, words, window);
     return -1;
   }
+  // Masked scores are -inf before they are scaled and maxima are taken before it too, so the scale has to be positive; it
+  // stays a normal number after the e4m3 path's powers of two, 2^-100 to 2^100.
+  if (!(scale >= 0.99e-7f && scale <= 1.01e4f)) {
+    set_last_error("afb_tree_attention: the scale is a positive number from 1e-7 to 1e4, not %g", static_cast<double>(scale));
+    return -1;
+  }
   const auto odd = [](const void* x, int to) { return (reinterpret_cast<uintptr_t>(x) & (to - 1)) != 0; };
   if (odd(q, 16) || odd(out, 16) || odd(k_cache, 16) || odd(v_cache, 16) || odd(scratch, 16) || q_stride % 8 || out_stride % 8) {
     set_last_error("afb_tree_attention: q, out and the caches start on 16 bytes, token strides are multiples of 8 elements");

@@ -148,3 +148,18 @@ def test_refusals_name_what_is_wrong():
         TR.tree_accept(t, t, t, caches=[(k, k, i32([[0, 1]]))])
     with pytest.raises(ValueError, match="contiguous"):
         TR.tree_accept(t, t, t, caches=[(k[:, :2], k[:, :2], t)])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), -float("inf"), 1e-8, 1e5])
+def test_scales_that_are_not_positive_numbers_are_refused(scale):
+    c = Case([9, 70], [3, 2], 4, 2, 64, 8)
+    args, kw = c.args("cpu")
+    with pytest.raises(ValueError, match="scale must be a positive number"):
+        TR.tree_attention(*args, scale=scale, **kw)
+
+
+@pytest.mark.parametrize("scale", [1e-7, 1.0, 1e4])
+def test_scales_at_the_ends_of_their_range(scale):
+    c = Case([9, 70], [3, 2], 4, 2, 64, 8)
+    args, kw = c.args("cpu")
+    assert torch.isfinite(TR.tree_attention(*args, scale=scale, **kw)).all()
