@@ -67,6 +67,7 @@ def _stream(*tensors) -> int:
 
 
 _i32 = torch.int32
+_INT_MAX = 2 ** 31 - 1
 _CACHES = (torch.bfloat16, torch.float8_e4m3fn, torch.float32)
 
 
@@ -181,8 +182,9 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     number from 1e-7 to 1e4.
 
     ``max_q_len`` bounds ``q_lens`` and ``max_kv`` (0: what the block table can hold) bounds ``kv_lens``; both size the
-    launch.  Rows of ``out`` that belong to no sequence are left as they were; in a new output those behind the last
-    sequence are zero."""
+    launch, and a length past them is reported through the status word.  A window of ``max_kv`` keys or more is none.
+    Rows of ``out`` that belong to no sequence are left as they were; in a new output those behind the last sequence are
+    zero."""
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, D], got {list(q.shape)}")
     T, Hq, D = q.shape
@@ -244,9 +246,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     if B == 0:
         return y.zero_() if out is None else out
     # The keys of a sequence may be shared out over several CTAs, whose partial rows (32 bits) are joined in the end.
-    reach = block_tables.shape[1] * page
-    if max_kv:
-        reach = min(reach, max_kv)
+    reach = min(block_tables.shape[1] * page, max_kv or _INT_MAX, _INT_MAX)
+    window, max_q_len = min(window, _INT_MAX), min(max_q_len, T, nodes)
     kv8 = 0 if kind is torch.bfloat16 else 1
     lib = _lib()
     floats = lib.afb_tree_attention_scratch(B, T, Hq, Hkv, D, kv8, page, nodes, window, max_q_len, reach)

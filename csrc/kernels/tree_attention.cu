@@ -28,7 +28,9 @@ struct TreeAttnParams {
   long depth_stride;
   __nv_bfloat16* out;
   long out_stride;
-  int T, Hq, Hkv, D, window;
+  int T, Hq, Hkv, D;
+  int window;                // 0: none, also for one that reaches every key of max_kv
+  int max_kv;                // what the caller says that no kv_len passes
   int zero_tail;             // rows behind the last sequence become zero
   float scale_log2;
   int B, max_q, box_rows, page_shift;         // log2(page), -1 when page is no power of two
@@ -56,7 +58,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnParams& p, int b) {
   s.tree_len = max(0, min(min(tl, s.kv_len), p.nodes));
   s.q_len = min(min(s.q_len, s.tree_len), p.max_q);
   s.base = s.kv_len - s.tree_len;
-  if (s.q_start != q0 || s.q_len != ql || s.kv_len != kv || s.tree_len != tl) status_set(kStatusBadIndex);
+  if (s.q_start != q0 || s.q_len != ql || s.kv_len != kv || s.tree_len != tl || kv > p.max_kv) status_set(kStatusBadIndex);
   return s;
 }
 
@@ -1392,6 +1394,9 @@ int launch_mma(const TreeAttnParams& p, int wr, long ctas, cudaStream_t stream) 
                  : wr == 2 ? launch_mma<DP, 2, KV8>(p, ctas, stream) : launch_mma<DP, 4, KV8>(p, ctas, stream);
 }
 
+// A window that reaches the first key of the longest sequence masks nothing: positions lie below max_kv.
+inline int real_window(int window, int max_kv) { return window > 0 && window < max_kv ? window : 0; }
+
 // Sizes of a launch: what follows from the shapes alone, so that the caller can provide the partial rows.
 struct TreeLaunch {
   bool tc;
@@ -1422,8 +1427,8 @@ inline TreeLaunch tree_launch(int B, int T, int Hq, int Hkv, int D, int kv8, int
   }
   t.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   t.row_tiles = rows > 0 ? (rows + 16 * t.wr - 1) / (16 * t.wr) : 1;
-  const int reach = window > 0 && window + nodes + 63 < max_kv ? window + nodes + 63 : max_kv;
-  const int tiles = reach / kKeys + 1;
+  const long reach = window > 0 ? static_cast<long>(window) + nodes + 63 : max_kv;     // (64 bits: the sum may pass 2^31)
+  const int tiles = static_cast<int>(reach < max_kv ? reach : max_kv) / kKeys + 1;
   t.chunk = pick_chunk(static_cast<long>(B) * Hkv * t.row_tiles, tiles, device_sm_count() * (D <= 64 ? 3 : D <= 128 ? 2 : 1));
   t.splits = (tiles + t.chunk - 1) / t.chunk;
   t.part_rows = static_cast<long>(T) * Hq;
@@ -1440,7 +1445,7 @@ long afb_tree_attention_scratch(int B, int T, int Hq, int Hkv, int D, int kv8, i
                                 int max_q_len, int max_kv) {
   using namespace afb;
   if (B <= 0 || Hkv <= 0 || Hq < Hkv || page <= 0 || max_q_len < 0 || max_kv < 0) return 0;
-  return tree_launch(B, T, Hq, Hkv, D, kv8, page, nodes, window, max_q_len, max_kv).scratch;
+  return tree_launch(B, T, Hq, Hkv, D, kv8, page, nodes, real_window(window, max_kv), max_q_len, max_kv).scratch;
 }
 
 int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const void* v_cache, int kv8, int num_blocks,
@@ -1469,6 +1474,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
     set_last_error("afb_tree_attention: q, out and the caches start on 16 bytes, token strides are multiples of 8 elements");
     return -1;
   }
+  window = real_window(window, max_kv);
   const TreeLaunch t = tree_launch(B, T, Hq, Hkv, D, kv8, page, nodes, window, max_q_len, max_kv);
   const long ctas = t.tc ? static_cast<long>(t.groups) * t.heads * t.row_tiles : static_cast<long>(B) * t.splits * Hkv * t.row_tiles;
   // tiles are counted in 32 bits on the device
@@ -1480,7 +1486,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   }
   TreeAttnParams p{static_cast<const __nv_bfloat16*>(q), q_stride, k_cache, v_cache, tables, table_stride, max_blocks, page,
                    num_blocks, q_starts, q_lens, kv_lens, tree_lens, masks, mask_stride, nodes, words, depths, depth_stride,
-                   static_cast<__nv_bfloat16*>(out), out_stride, T, Hq, Hkv, D, window > 0 ? window : 0, zero_tail,
+                   static_cast<__nv_bfloat16*>(out), out_stride, T, Hq, Hkv, D, window, max_kv, zero_tail,
                    scale * 1.4426950408889634f};
   p.B = B;
   p.max_q = max_q_len;
