@@ -183,8 +183,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
 
     ``max_q_len`` bounds ``q_lens`` and ``max_kv`` (0: what the block table can hold) bounds ``kv_lens``; both size the
     launch, and a length past them is reported through the status word.  A window of ``max_kv`` keys or more is none.
-    Rows of ``out`` that belong to no sequence are left as they were; in a new output those behind the last sequence are
-    zero."""
+    The sequences' rows may lie in any order but do not overlap.  Rows of ``out`` that belong to no sequence are left as
+    they were; in a new output they are zero."""
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, D], got {list(q.shape)}")
     T, Hq, D = q.shape

@@ -31,10 +31,11 @@ struct TreeAttnParams {
   int T, Hq, Hkv, D;
   int window;                // 0: none, also for one that reaches every key of max_kv
   int max_kv;                // what the caller says that no kv_len passes
-  int zero_tail;             // rows behind the last sequence become zero
+  int zero_rest;             // rows of no sequence become zero
   float scale_log2;
   int B, max_q, box_rows, page_shift;         // log2(page), -1 when page is no power of two
   int row_tiles;             // of a KV head
+  int ctas;                  // mma.sync: those that have keys
   int splits, chunk;         // chunks of a sequence at most; 64-key tiles of a chunk
   int groups;                // tcgen05: pieces of the line of tiles
   int heads, blocks;         // KV heads of a block, blocks
@@ -85,11 +86,36 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Columns col .. col + n - 1 (multiples of 8) of the rows behind the last sequence: this thread's, of `threads`.
-__device__ __forceinline__ void zero_rows(const TreeAttnParams& p, const TreeSeq& s, int col, int n, long threads, long me) {
-  for (long x = me; x < (p.T - s.q_start - s.q_len) * static_cast<long>(n / 8); x += threads)
-    *reinterpret_cast<uint4*>(p.out + (s.q_start + s.q_len + x / (n / 8)) * p.out_stride + col + x % (n / 8) * 8) =
-        make_uint4(0, 0, 0, 0);
+// Zeros in columns col .. col + n - 1 (multiples of 8) of the rows that belong to no sequence, by warp w of `warps`.  Starts
+// may be in any order.  Rows that lie next to one another, whichever is first, are as many as the largest end says, and then
+// only those behind it are left; otherwise every row is looked up.
+__device__ __forceinline__ void zero_unused(const TreeAttnParams& p, int col, int n, long warps, long w) {
+  const int lane = threadIdx.x & 31, cols = n / 8;
+  long used = 0, end = 0;
+  for (int b = lane; b < p.B; b += 32) {
+    const TreeSeq s = tree_seq(p, b);
+    used += s.q_len;
+    if (s.q_len > 0) end = max(end, static_cast<long>(s.q_start) + s.q_len);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    used += __shfl_xor_sync(0xffffffffu, used, o);
+    end = max(end, __shfl_xor_sync(0xffffffffu, end, o));
+  }
+  const auto zero = [&](long row, int c) {
+    *reinterpret_cast<uint4*>(p.out + row * p.out_stride + col + c * 8) = make_uint4(0, 0, 0, 0);
+  };
+  for (long x = w * 32 + lane; x < (p.T - end) * cols; x += warps * 32) zero(end + x / cols, static_cast<int>(x % cols));
+  if (used == end) return;
+  for (long row = w; row < end; row += warps) {
+    bool mine = false;
+    for (int b = lane; b < p.B; b += 32) {
+      const TreeSeq s = tree_seq(p, b);
+      mine |= row >= s.q_start && row < static_cast<long>(s.q_start) + s.q_len;
+    }
+    if (__any_sync(0xffffffffu, mine)) continue;
+    for (int c = lane; c < cols; c += 32) zero(row, c);
+  }
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -272,15 +298,18 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
   const int wr = warp % WR, wk = warp / WR;
   griddep_launch();
   griddep_wait();
+  const int G = p.Hq / p.Hkv;
+  if (static_cast<int>(blockIdx.x) >= p.ctas) {      // a CTA per KV head behind the others
+    zero_unused(p, (blockIdx.x - p.ctas) * G * p.D, G * p.D, 4, warp);
+    return;
+  }
   // row tiles of one head next to one another: they share the keys in L2
   int idx = blockIdx.x;
   const int rt = idx % p.row_tiles; idx /= p.row_tiles;
   const int hk = idx % p.Hkv; idx /= p.Hkv;
   const int split = idx % p.splits, b = idx / p.splits;
-  const int G = p.Hq / p.Hkv;
   const TreeSeq s = tree_seq(p, b);
   const int rows = s.q_len * G, row0 = rt * 16 * WR;
-  if (p.zero_tail && b == p.B - 1 && split == 0 && rt == 0) zero_rows(p, s, hk * G * p.D, G * p.D, 128, threadIdx.x);
   const TreeTiles tt = tree_tiles(p, s);
   const int t0 = tt.lo + split * p.chunk, t1 = min(tt.hi, t0 + p.chunk);
   const int ntiles = t1 - t0;
@@ -569,7 +598,7 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 //   13, 14  TMA of K and of V, one box per piece of a page (the largest power of two of rows that divides the page size,
 //        at most 128) and 128 bytes of columns; zeros come from outside the tensor for D that fills no box and for block
 //        ids that are none.  K tiles are free again once their scores are there, long before the V tile of the same keys.
-//        Warp 14 has the zeros behind the last sequence, too.
+//        Warp 14 has the zeros of the rows that no sequence has, too.
 // Tensor memory: three score tiles (the next scores are there before this tile's weights are) and O.
 //
 // e4m3 caches are expanded to fp16, which holds every e4m3 value exactly and takes one conversion instruction per two
@@ -801,15 +830,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     per = max(1, (line + p.groups - 1) / p.groups);
     if (p.B <= kTcThreads) break;
   }
-  const auto zero_tail = [&] {
-    if (p.zero_tail) zero_rows(p, tree_seq(p, p.B - 1), 0, p.Hq * p.D, 32l * gridDim.x, 32l * blockIdx.x + lane);
+  const auto zero_rest = [&] {                     // by a whole warp
+    if (p.zero_rest) zero_unused(p, 0, p.Hq * p.D, gridDim.x, blockIdx.x);
   };
   TcWalk walk;
   walk.sub = blockIdx.x / p.row_tiles % p.heads;
   walk.at = group * per;
   walk.end = min(line, walk.at + per);
   if (walk.at >= line) {                          // whole CTA, nothing allocated
-    if (warp == 14) zero_tail();
+    if (warp == 14) zero_rest();
     return;
   }
   if (warp == 12) {
@@ -1171,7 +1200,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!alive)                                  // nothing may land in this CTA's shared memory after it has gone
         for (int i = max(0, j - L::kRaw); i < j; ++i)
           mbar_wait(full(v, i % L::kRaw), (i / L::kRaw) & 1, kStatusTmaWaitTimeout);
-      if (v) zero_tail();
+      __syncwarp();
+      if (v) zero_rest();
     } else if (warp == 12 && lane == 0) {
       // -------------------------------------------------------------- the MMAs
       constexpr uint32_t kind = KV8 ? ~((1u << 7) | (1u << 10)) : ~0u;     // operands fp16 or bf16
@@ -1452,7 +1482,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
                        int page, const int* tables, long table_stride, int max_blocks, const int* q_starts,
                        const int* q_lens, const int* kv_lens, const int* tree_lens, const int* masks, long mask_stride,
                        int nodes, int words, const int* depths, long depth_stride, void* out, long out_stride, int B,
-                       int T, int Hq, int Hkv, int D, int max_q_len, int max_kv, int window, int zero_tail, float scale,
+                       int T, int Hq, int Hkv, int D, int max_q_len, int max_kv, int window, int zero_rest, float scale,
                        float* scratch, long scratch_floats, cudaStream_t stream) {
   using namespace afb;
   if (B <= 0 || T <= 0) return 0;
@@ -1478,15 +1508,16 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   const TreeLaunch t = tree_launch(B, T, Hq, Hkv, D, kv8, page, nodes, window, max_q_len, max_kv);
   const long ctas = t.tc ? static_cast<long>(t.groups) * t.heads * t.row_tiles : static_cast<long>(B) * t.splits * Hkv * t.row_tiles;
   // tiles are counted in 32 bits on the device
+  const long grid = ctas + (zero_rest && !t.tc ? Hkv : 0);
   const long line = (static_cast<long>(max_blocks) * page / kKeys + 1) * B * Hkv;
-  if (t.scratch > scratch_floats || (t.scratch && !scratch) || ctas > 0x7fffffffl || line > 0x7fffffffl) {
+  if (t.scratch > scratch_floats || (t.scratch && !scratch) || grid > 0x7fffffffl || line > 0x7fffffffl) {
     set_last_error("afb_tree_attention: %ld floats of scratch are needed, %ld given (or too many tiles: %ld)", t.scratch,
                    scratch_floats, line);
     return -1;
   }
   TreeAttnParams p{static_cast<const __nv_bfloat16*>(q), q_stride, k_cache, v_cache, tables, table_stride, max_blocks, page,
                    num_blocks, q_starts, q_lens, kv_lens, tree_lens, masks, mask_stride, nodes, words, depths, depth_stride,
-                   static_cast<__nv_bfloat16*>(out), out_stride, T, Hq, Hkv, D, window, max_kv, zero_tail,
+                   static_cast<__nv_bfloat16*>(out), out_stride, T, Hq, Hkv, D, window, max_kv, zero_rest,
                    scale * 1.4426950408889634f};
   p.B = B;
   p.max_q = max_q_len;
@@ -1494,6 +1525,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   for (int sh = 0; sh < 31; ++sh)
     if (page == 1 << sh) p.page_shift = sh;
   p.row_tiles = t.row_tiles;
+  p.ctas = static_cast<int>(ctas);
   p.splits = t.tc ? 1 << 20 : t.splits;
   p.chunk = t.tc ? 1 << 20 : t.chunk;
   p.groups = t.groups;
@@ -1508,11 +1540,11 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
     rc = D <= 64 ? (kv8 ? launch_tc<64, true>(p, ctas, stream) : launch_tc<64, false>(p, ctas, stream))
                  : kv8 ? launch_tc<128, true>(p, ctas, stream) : launch_tc<128, false>(p, ctas, stream);
   else if (kv8)
-    rc = D <= 64 ? launch_mma<64, true>(p, t.wr, ctas, stream)
-                 : D <= 128 ? launch_mma<128, true>(p, t.wr, ctas, stream) : launch_mma<256, true>(p, t.wr, ctas, stream);
+    rc = D <= 64 ? launch_mma<64, true>(p, t.wr, grid, stream)
+                 : D <= 128 ? launch_mma<128, true>(p, t.wr, grid, stream) : launch_mma<256, true>(p, t.wr, grid, stream);
   else
-    rc = D <= 64 ? launch_mma<64, false>(p, t.wr, ctas, stream)
-                 : D <= 128 ? launch_mma<128, false>(p, t.wr, ctas, stream) : launch_mma<256, false>(p, t.wr, ctas, stream);
+    rc = D <= 64 ? launch_mma<64, false>(p, t.wr, grid, stream)
+                 : D <= 128 ? launch_mma<128, false>(p, t.wr, grid, stream) : launch_mma<256, false>(p, t.wr, grid, stream);
   if (rc) return rc;
   const long out_rows = static_cast<long>(max_q_len) * Hq;
   if (t.tc && t.groups > 1)
