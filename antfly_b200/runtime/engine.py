@@ -473,15 +473,19 @@ class LLMEngine:
 
     def step(self) -> int:
         """Run one scheduler step.  Returns the number of tokens produced."""
+        speculate = False
         if self.draft is not None and not any(r.params.grammar is not None and not r.finished
                                               for r in self.reqs.values()):
             snap = self.sched.snapshot()
-            if snap["decode"] > 0 and snap["waiting"] + snap["prefill"] == 0 and not any(
-                    r.soft_rows is not None for r in self.reqs.values()):
-                return self._spec_round()
+            speculate = snap["decode"] > 0 and snap["waiting"] + snap["prefill"] == 0 and not any(
+                r.soft_rows is not None for r in self.reqs.values())
         items = self.sched.claim_step()
         if not items:
             return 0
+        if speculate:
+            produced = self._spec_round(items)
+            if produced is not None:
+                return produced
         t_start = time.perf_counter()
         reqs = [self.reqs[it.request_id] for it in items]
         try:
@@ -582,18 +586,36 @@ class LLMEngine:
         return N - M
 
     # ------------------------------------------------------------------------------------------------
-    def _spec_round(self) -> int:
+    def _spec_fits(self, items: List[StepItem], n: int, n_draft: int) -> bool:
+        """Whether n more tokens of every sequence fit its block table and the pool, and n_draft the pool of a separate
+        draft behind what that has to catch up with.  Cached prefixes give way where that is enough."""
+        pages = lambda tokens: (tokens + self.page - 1) // self.page
+        if max(it.kv_before for it in items) + n > self.max_blocks * self.page:
+            return False
+        if self.draft_cache is not None:
+            d = self.draft_cache.alloc
+            held = [pages(d.length(it.request_id)) if self.reqs[it.request_id].draft_attached else 0 for it in items]
+            if sum(max(0, pages(it.kv_before + n_draft) - h) for it, h in zip(items, held)) > d.free_blocks:
+                return False
+        alloc = self.cache.alloc
+        need = sum(pages(it.kv_before + n) - pages(it.kv_before) for it in items)
+        if need > alloc.free_blocks and self.prefix is not None:
+            live = sum(pages(alloc.length(r.rid)) for r in self.reqs.values() if not r.finished)
+            while live + need <= self.cache.num_blocks and need > alloc.free_blocks and self.prefix.evict_one():
+                pass
+        return need <= alloc.free_blocks
+
+    def _spec_round(self, items: List[StepItem]) -> Optional[int]:
         """One speculative round for every decoding sequence: K greedy draft steps on the shallow model (which
         shares the target's first layers and their KV cache), one target pass over K+1 positions, verify/accept,
-        KV rollback of the rejected tail."""
-        items = self.sched.claim_step()
-        if not items:
-            return 0
+        KV rollback of the rejected tail.  None, with nothing done, when there is no room for the drafts."""
         reqs = [self.reqs[it.request_id] for it in items]
-        if self._tree is not None and max(it.kv_before for it in items) + self._tree["nodes"] <= self.max_blocks * self.page:
+        if self._tree is not None and self._spec_fits(items, self._tree["nodes"], self._tree["levels"][-1][0]):
             return self._tree_round(items, reqs)
         # Draft length of the round: the smallest of what the requests ask for (default: the engine's), 1..16.
         K = max(1, min(16, min((r.params.speculative_k or self.spec_k) for r in reqs)))
+        if not self._spec_fits(items, K + 1, K):
+            return None
         B = len(items)
         alloc = self.cache.alloc
         separate = self.draft_cache is not None
@@ -706,24 +728,10 @@ class LLMEngine:
             self._draft_catch_up(items, reqs)
         n_draft = levels[-1][0]                       # the draft model is not asked for what follows the last level
 
-        def reserve(alloc, n):
-            for i, r in enumerate(rids):
-                try:
-                    alloc.append(r, n)
-                except KvOutOfBlocks:
-                    for r2, b2 in zip(rids[:i], base):
-                        alloc.truncate(r2, b2)
-                    self.sched.fail_step()
-                    raise
-
-        reserve(self.cache.alloc, nodes)
-        if separate:
-            try:
-                reserve(self.draft_cache.alloc, n_draft)
-            except KvOutOfBlocks:
-                for r, b in zip(rids, base):
-                    self.cache.alloc.truncate(r, b)
-                raise
+        for r in rids:
+            self.cache.alloc.append(r, nodes)
+            if separate:
+                self.draft_cache.alloc.append(r, n_draft)
         blocks = self._blocks_of(rids)
         dblocks = self._blocks_of(rids, self.draft_cache.alloc) if separate else blocks[:0]
         last = [r.out[-1] for r in reqs]

@@ -94,6 +94,44 @@ def test_an_exhausted_pool_leaves_the_sequences_as_they_were():
     assert eng.cache.alloc.length(rid) == len(r.prompt) + len(r.out) - 1
 
 
+DRAFTS = [lambda: dict(draft_layers=1), lambda: dict(draft_model=_model()), lambda: dict(draft_model=_model(), draft_num_blocks=3)]
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("form", [dict(spec_tree=(8, 2)), dict(spec_tree=(2, 1)), dict(spec_k=4)])
+def test_a_pool_that_holds_the_continuation_but_not_the_drafts(draft, form):
+    """Four blocks hold the 63 tokens of a request to the last; rounds whose drafts do not fit them, or a separate draft's
+    pool, give way to chains and in the end to plain steps."""
+    sp, prompt = SamplingParams(max_tokens=24), [PROMPTS[0] * 2]
+    plain = [r.token_ids for r in _engine(num_blocks=4).generate(prompt, sp)]
+    eng = _engine(num_blocks=4, **{**draft(), **form})
+    assert [r.token_ids for r in eng.generate(prompt, sp)] == plain and len(plain[0]) == 24
+    assert eng.cache.alloc.free_blocks == 4
+    assert eng.draft_cache is None or eng.draft_cache.alloc.free_blocks == eng.draft_cache.num_blocks
+
+
+@pytest.mark.parametrize("form", [dict(spec_tree=(4, 2)), dict(spec_k=4)])
+def test_cached_prefixes_give_way_to_drafts(form):
+    """The first prompts' blocks stay cached until the pool is full; the last request still speculates."""
+    sp, prompts = SamplingParams(max_tokens=12), [[i + 1] * 32 for i in range(3)] + [PROMPTS[0]]
+    plain = [_engine(num_blocks=8).generate([p], sp)[0].token_ids for p in prompts]
+    eng = _engine(num_blocks=8, draft_layers=1, prefix_cache=True, **form)
+    got = []
+    for p in prompts:
+        before = eng.spec.rounds
+        got.append(eng.generate([p], sp)[0].token_ids)
+        assert eng.spec.rounds > before
+    assert got == plain and eng.prefix.evictions > 0
+
+
+def test_a_chain_at_the_end_of_the_block_table_gives_way_to_plain_steps(plain):
+    eng = LLMEngine(_model(), num_blocks=16, page=16, max_batch=4, max_step_tokens=64, use_cuda_graph=False, max_seq_len=48,
+                    draft_layers=1, spec_k=4)
+    want = LLMEngine(_model(), num_blocks=16, page=16, max_batch=4, max_step_tokens=64, use_cuda_graph=False, max_seq_len=48)
+    sp = SamplingParams(max_tokens=28)
+    assert eng.generate([PROMPTS[0]], sp)[0].token_ids == want.generate([PROMPTS[0]], sp)[0].token_ids
+
+
 def test_sampled_requests_run_over_trees():
     sp = SamplingParams(max_tokens=6, temperature=0.8, top_k=20, repetition_penalty=1.1, seed=3)
     out = _engine(draft_layers=1, spec_tree=(2, 2)).generate(PROMPTS[:2], sp)
