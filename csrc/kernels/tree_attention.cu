@@ -35,7 +35,6 @@ struct TreeAttnParams {
   float scale_log2;
   int B, max_q, box_rows, page_shift;         // log2(page), -1 when page is no power of two
   int row_tiles;             // of a KV head
-  int ctas;                  // mma.sync: those that have keys
   int splits, chunk;         // chunks of a sequence at most; 64-key tiles of a chunk
   int groups;                // tcgen05: pieces of the line of tiles
   int heads, blocks;         // KV heads of a block, blocks
@@ -86,35 +85,30 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Zeros in columns col .. col + n - 1 (multiples of 8) of the rows that belong to no sequence, by warp w of `warps`.  Starts
-// may be in any order.  Rows that lie next to one another, whichever is first, are as many as the largest end says, and then
-// only those behind it are left; otherwise every row is looked up.
-__device__ __forceinline__ void zero_unused(const TreeAttnParams& p, int col, int n, long warps, long w) {
-  const int lane = threadIdx.x & 31, cols = n / 8;
-  long used = 0, end = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    const TreeSeq s = tree_seq(p, b);
-    used += s.q_len;
-    if (s.q_len > 0) end = max(end, static_cast<long>(s.q_start) + s.q_len);
+// Zeros in the rows that belong to no sequence and follow those of sequence b (for the first also in front of all), columns
+// col .. col + n - 1 (multiples of 8): this thread's, of `threads`.  Starts may be in any order.  Where every sequence begins
+// at the end of the one before it and the last ends at T, there is nothing to do and that shows from one more load (`next`,
+// which is best on its way with the others); otherwise the next start is looked up.
+__device__ __forceinline__ int next_start(const TreeAttnParams& p, int b) { return b + 1 < p.B ? p.q_starts[b + 1] : p.T; }
+__device__ __forceinline__ void zero_gap(const TreeAttnParams& p, const TreeSeq& s, int next, int b, int col, int n,
+                                         int threads, int me) {
+  const int end = s.q_start + s.q_len;
+  const bool front = b == 0 && (s.q_start > 0 || s.q_len == 0), behind = s.q_len > 0 && next != end;
+  if (!front && !behind) return;
+  int first = p.T, after = p.T;                    // start of all rows that sequences have, of those from `end` on
+  for (int c = threadIdx.x & 31; c < p.B; c += 32) {
+    const TreeSeq t = tree_seq(p, c);
+    if (t.q_len == 0) continue;
+    first = min(first, t.q_start);
+    if (t.q_start >= end) after = min(after, t.q_start);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    used += __shfl_xor_sync(0xffffffffu, used, o);
-    end = max(end, __shfl_xor_sync(0xffffffffu, end, o));
-  }
-  const auto zero = [&](long row, int c) {
-    *reinterpret_cast<uint4*>(p.out + row * p.out_stride + col + c * 8) = make_uint4(0, 0, 0, 0);
-  };
-  for (long x = w * 32 + lane; x < (p.T - end) * cols; x += warps * 32) zero(end + x / cols, static_cast<int>(x % cols));
-  if (used == end) return;
-  for (long row = w; row < end; row += warps) {
-    bool mine = false;
-    for (int b = lane; b < p.B; b += 32) {
-      const TreeSeq s = tree_seq(p, b);
-      mine |= row >= s.q_start && row < static_cast<long>(s.q_start) + s.q_len;
-    }
-    if (__any_sync(0xffffffffu, mine)) continue;
-    for (int c = lane; c < cols; c += 32) zero(row, c);
+  first = front ? __reduce_min_sync(0xffffffffu, first) : 0;
+  after = behind ? __reduce_min_sync(0xffffffffu, after) : end;
+  const int cols = n / 8;
+  for (long x = me; x < static_cast<long>(first + after - end) * cols; x += threads) {
+    const long row = x / cols;
+    *reinterpret_cast<uint4*>(p.out + (row < first ? row : row - first + end) * p.out_stride + col + x % cols * 8) =
+        make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -298,18 +292,16 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
   const int wr = warp % WR, wk = warp / WR;
   griddep_launch();
   griddep_wait();
-  const int G = p.Hq / p.Hkv;
-  if (static_cast<int>(blockIdx.x) >= p.ctas) {      // a CTA per KV head behind the others
-    zero_unused(p, (blockIdx.x - p.ctas) * G * p.D, G * p.D, 4, warp);
-    return;
-  }
   // row tiles of one head next to one another: they share the keys in L2
   int idx = blockIdx.x;
   const int rt = idx % p.row_tiles; idx /= p.row_tiles;
   const int hk = idx % p.Hkv; idx /= p.Hkv;
   const int split = idx % p.splits, b = idx / p.splits;
+  const int G = p.Hq / p.Hkv;
+  const int next = next_start(p, b);
   const TreeSeq s = tree_seq(p, b);
   const int rows = s.q_len * G, row0 = rt * 16 * WR;
+  if (p.zero_rest && split == 0 && rt == 0) zero_gap(p, s, next, b, hk * G * p.D, G * p.D, 128, threadIdx.x);
   const TreeTiles tt = tree_tiles(p, s);
   const int t0 = tt.lo + split * p.chunk, t1 = min(tt.hi, t0 + p.chunk);
   const int ntiles = t1 - t0;
@@ -598,7 +590,6 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 //   13, 14  TMA of K and of V, one box per piece of a page (the largest power of two of rows that divides the page size,
 //        at most 128) and 128 bytes of columns; zeros come from outside the tensor for D that fills no box and for block
 //        ids that are none.  K tiles are free again once their scores are there, long before the V tile of the same keys.
-//        Warp 14 has the zeros of the rows that no sequence has, too.
 // Tensor memory: three score tiles (the next scores are there before this tile's weights are) and O.
 //
 // e4m3 caches are expanded to fp16, which holds every e4m3 value exactly and takes one conversion instruction per two
@@ -830,17 +821,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     per = max(1, (line + p.groups - 1) / p.groups);
     if (p.B <= kTcThreads) break;
   }
-  const auto zero_rest = [&] {                     // by a whole warp
-    if (p.zero_rest) zero_unused(p, 0, p.Hq * p.D, gridDim.x, blockIdx.x);
-  };
   TcWalk walk;
   walk.sub = blockIdx.x / p.row_tiles % p.heads;
   walk.at = group * per;
   walk.end = min(line, walk.at + per);
-  if (walk.at >= line) {                          // whole CTA, nothing allocated
-    if (warp == 14) zero_rest();
-    return;
-  }
+  if (walk.at >= line) return;                    // whole CTA, nothing allocated
   if (warp == 12) {
     tmem_alloc(tmem_slot, L::kTmem);
     tmem_relinquish();
@@ -1200,8 +1185,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!alive)                                  // nothing may land in this CTA's shared memory after it has gone
         for (int i = max(0, j - L::kRaw); i < j; ++i)
           mbar_wait(full(v, i % L::kRaw), (i / L::kRaw) & 1, kStatusTmaWaitTimeout);
-      __syncwarp();
-      if (v) zero_rest();
     } else if (warp == 12 && lane == 0) {
       // -------------------------------------------------------------- the MMAs
       constexpr uint32_t kind = KV8 ? ~((1u << 7) | (1u << 10)) : ~0u;     // operands fp16 or bf16
@@ -1283,12 +1266,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // Joins the (sequence, head)s of the kernel above that lie on several pieces of the line.  A thread takes eight columns of
-// rows of one sequence; the sequence's place on the line is summed up by the block.
+// rows of one sequence; the sequence's place on the line is summed up by the block.  It has the zeros of the rows that no
+// sequence has, too.
 __global__ void __launch_bounds__(256) tree_attn_tc_join_kernel(const __grid_constant__ TreeAttnParams p) {
   __shared__ int red[8];
   griddep_launch();
   griddep_wait();
   const int b = blockIdx.y;
+  const int next = next_start(p, b);
+  const TreeSeq s = tree_seq(p, b);
   __shared__ int s_start;
   int start = 0, line = 0;
   for (int b0 = 0; b0 < p.B; b0 += 256) {
@@ -1302,7 +1288,7 @@ __global__ void __launch_bounds__(256) tree_attn_tc_join_kernel(const __grid_con
   __syncthreads();
   start = s_start;
   const int per = max(1, (line + p.groups - 1) / p.groups);
-  const TreeSeq s = tree_seq(p, b);
+  if (p.zero_rest) zero_gap(p, s, next, b, 0, p.Hq * p.D, gridDim.x * 256, blockIdx.x * 256 + threadIdx.x);
   const int tiles = tc_tiles(s), G = p.Hq / p.Hkv, chunks = p.D / 8;
   for (int y = blockIdx.x * 256 + threadIdx.x; y < s.q_len * p.Hq * chunks; y += gridDim.x * 256) {
     const int x = y / chunks, ch = y - x * chunks;
@@ -1508,9 +1494,8 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   const TreeLaunch t = tree_launch(B, T, Hq, Hkv, D, kv8, page, nodes, window, max_q_len, max_kv);
   const long ctas = t.tc ? static_cast<long>(t.groups) * t.heads * t.row_tiles : static_cast<long>(B) * t.splits * Hkv * t.row_tiles;
   // tiles are counted in 32 bits on the device
-  const long grid = ctas + (zero_rest && !t.tc ? Hkv : 0);
   const long line = (static_cast<long>(max_blocks) * page / kKeys + 1) * B * Hkv;
-  if (t.scratch > scratch_floats || (t.scratch && !scratch) || grid > 0x7fffffffl || line > 0x7fffffffl) {
+  if (t.scratch > scratch_floats || (t.scratch && !scratch) || ctas > 0x7fffffffl || line > 0x7fffffffl) {
     set_last_error("afb_tree_attention: %ld floats of scratch are needed, %ld given (or too many tiles: %ld)", t.scratch,
                    scratch_floats, line);
     return -1;
@@ -1525,7 +1510,6 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   for (int sh = 0; sh < 31; ++sh)
     if (page == 1 << sh) p.page_shift = sh;
   p.row_tiles = t.row_tiles;
-  p.ctas = static_cast<int>(ctas);
   p.splits = t.tc ? 1 << 20 : t.splits;
   p.chunk = t.tc ? 1 << 20 : t.chunk;
   p.groups = t.groups;
@@ -1540,14 +1524,14 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
     rc = D <= 64 ? (kv8 ? launch_tc<64, true>(p, ctas, stream) : launch_tc<64, false>(p, ctas, stream))
                  : kv8 ? launch_tc<128, true>(p, ctas, stream) : launch_tc<128, false>(p, ctas, stream);
   else if (kv8)
-    rc = D <= 64 ? launch_mma<64, true>(p, t.wr, grid, stream)
-                 : D <= 128 ? launch_mma<128, true>(p, t.wr, grid, stream) : launch_mma<256, true>(p, t.wr, grid, stream);
+    rc = D <= 64 ? launch_mma<64, true>(p, t.wr, ctas, stream)
+                 : D <= 128 ? launch_mma<128, true>(p, t.wr, ctas, stream) : launch_mma<256, true>(p, t.wr, ctas, stream);
   else
-    rc = D <= 64 ? launch_mma<64, false>(p, t.wr, grid, stream)
-                 : D <= 128 ? launch_mma<128, false>(p, t.wr, grid, stream) : launch_mma<256, false>(p, t.wr, grid, stream);
+    rc = D <= 64 ? launch_mma<64, false>(p, t.wr, ctas, stream)
+                 : D <= 128 ? launch_mma<128, false>(p, t.wr, ctas, stream) : launch_mma<256, false>(p, t.wr, ctas, stream);
   if (rc) return rc;
   const long out_rows = static_cast<long>(max_q_len) * Hq;
-  if (t.tc && t.groups > 1)
+  if (t.tc && (t.groups > 1 || zero_rest))
     AFB_CHECK_CUDA(launch_pdl(tree_attn_tc_join_kernel, dim3(static_cast<unsigned>((out_rows * (D / 8) + 255) / 256), B),
                               dim3(256), 0, stream, p));
   else if (!t.tc && t.splits > 1)
