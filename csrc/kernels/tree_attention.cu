@@ -1534,7 +1534,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
   if (t.tc && (t.groups > 1 || zero_rest))
     AFB_CHECK_CUDA(launch_pdl(tree_attn_tc_join_kernel, dim3(static_cast<unsigned>((out_rows * (D / 8) + 255) / 256), B),
                               dim3(256), 0, stream, p));
-  else if (!t.tc && t.splits > 1)
+  else if (!t.tc && t.splits > 1 && out_rows > 0)
     AFB_CHECK_CUDA(launch_pdl(tree_attn_join_kernel, dim3(static_cast<unsigned>((out_rows * (D / 4) + 127) / 128), B), dim3(128), 0,
                               stream, p));
   return 0;
