@@ -171,7 +171,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
                    max_kv: int = 0, scale: Optional[float] = None, window: int = 0,
                    depths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of packed tree nodes q [T, Hq, D] (bf16) over the paged cache [num_blocks, page, Hkv, D] (bf16 or e4m3;
-    a :class:`antfly_b200.ops.kv_quant.CodecLayer` too).  D is a multiple of 8 up to 256, Hq a multiple of Hkv.
+    a :class:`antfly_b200.ops.kv_quant.CodecLayer` too: fp8 as it lies, of the other codecs the pages of ``max_kv`` keys per
+    sequence are expanded to bf16 in every call).  D is a multiple of 8 up to 256, Hq a multiple of Hkv.
 
     The last ``tree_lens[b]`` of sequence b's ``kv_lens[b]`` keys are its tree's nodes and its ``q_lens[b]`` rows the last of
     those nodes (all of them in a verification pass, one level of them while drafting).  A row sees every key in front
@@ -188,22 +189,23 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, D], got {list(q.shape)}")
     T, Hq, D = q.shape
+    B = q_lens.numel()
+    q_starts, q_lens = _ints("q_starts", q_starts, B), _ints("q_lens", q_lens, B)
+    kv_lens, tree_lens = _ints("kv_lens", kv_lens, B), _ints("tree_lens", tree_lens, B)
+    block_tables = _ints("block_tables", block_tables, B, block_tables.shape[-1])
     if isinstance(k_cache, CodecLayer):
         if k_cache.codec == "fp8":
             shape = (k_cache.num_blocks, k_cache.page, k_cache.Hkv, D)
             k_cache, v_cache = (c.data.view(torch.float8_e4m3fn).view(shape) for c in (k_cache, v_cache))
         else:
-            k_cache, v_cache, block_tables = _expanded(k_cache, v_cache, block_tables, max_kv)
+            k_cache, v_cache, block_tables = _expanded(k_cache, v_cache, block_tables, kv_lens, max_kv)
     num_blocks, page, Hkv, Dk = k_cache.shape
-    B, kind = q_lens.numel(), k_cache.dtype
+    kind = k_cache.dtype
     if kind not in _CACHES or v_cache.dtype is not kind or v_cache.shape != k_cache.shape or Dk != D:
         raise ValueError(f"caches of one shape [blocks, page, Hkv, {D}] in bf16 or e4m3 are needed, got "
                          f"{k_cache.dtype} {list(k_cache.shape)} and {v_cache.dtype} {list(v_cache.shape)}")
     if D % 8 or not 8 <= D <= 256 or Hq % Hkv:
         raise ValueError(f"head width {D} (a multiple of 8 up to 256) or heads {Hq} over {Hkv} not supported")
-    q_starts, q_lens = _ints("q_starts", q_starts, B), _ints("q_lens", q_lens, B)
-    kv_lens, tree_lens = _ints("kv_lens", kv_lens, B), _ints("tree_lens", tree_lens, B)
-    block_tables = _ints("block_tables", block_tables, B, block_tables.shape[-1])
     masks = _ints("masks", masks, B, *masks.shape[1:]) if masks.dim() == 3 else _ints("masks", masks, B, None, None)
     nodes = masks.shape[1]
     if not 1 <= nodes <= MAX_NODES or masks.shape[2] != (nodes + 31) // 32:
@@ -263,18 +265,20 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     return y if out is None or y is out else out.copy_(y)
 
 
-def _expanded(k_cache, v_cache, block_tables, max_kv: int):
-    """Caches kept in another codec: the pages that the step can see, expanded to bf16, with a block table of their own."""
+def _expanded(k_cache, v_cache, block_tables, kv_lens, max_kv: int):
+    """Caches kept in another codec: the pages that the step can see, expanded to bf16, with a block table of their own.  A
+    block id that is none counts only where a key needs it."""
     page, Hkv, D = k_cache.page, k_cache.Hkv, k_cache.D
     nb = block_tables.shape[1]
     if max_kv > 0:
         nb = min(nb, (max_kv + page - 1) // page)
-    tab = block_tables[:, :nb]
-    rows = (tab.long().clamp_min(0) * page)[:, :, None] + torch.arange(page, device=tab.device)[None, None, :]
-    rows = rows.reshape(-1).int()
-    B = tab.shape[0]
+    B, dev = block_tables.shape[0], block_tables.device
+    key = torch.arange(nb * page, device=dev)
+    rows = (block_tables[:, :nb].long() * page)[:, :, None] + key[:page]
+    rows = rows.view(B, -1).clamp(-1, k_cache.num_blocks * page)         # ids that are none stay so in 32 bits
+    rows = torch.where(key < kv_lens[:, None], rows, 0).view(-1).int()
     kb, vb = (c.expand(rows).view(B * nb, page, Hkv, D) for c in (k_cache, v_cache))
-    return kb, vb, torch.arange(B * nb, dtype=torch.int32, device=tab.device).view(B, nb)
+    return kb, vb, torch.arange(B * nb, dtype=torch.int32, device=dev).view(B, nb)
 
 
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, lens: Optional[torch.Tensor] = None,

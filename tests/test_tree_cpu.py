@@ -163,3 +163,23 @@ def test_scales_at_the_ends_of_their_range(scale):
     c = Case([9, 70], [3, 2], 4, 2, 64, 8)
     args, kw = c.args("cpu")
     assert torch.isfinite(TR.tree_attention(*args, scale=scale, **kw)).all()
+
+
+def test_codec_caches_ask_nothing_of_table_entries_behind_the_last_key():
+    from antfly_b200.ops.kv_quant import CodecCache
+
+    c = Case([9, 30], [3, 2], 4, 2, 64, 8, seed=6)
+    k, v = (CodecCache("int8", 1, c.k.shape[0], 8, 2, 64, "cpu", value=x) for x in (False, True))
+    at = torch.arange(c.k.shape[0] * 8, dtype=torch.int32)
+    k[0].write(at, c.k.view(-1, 2, 64))
+    v[0].write(at, c.v.view(-1, 2, 64))
+    args, kw = c.args("cpu")
+    want = TR.tree_attention(args[0], k[0], v[0], *args[3:], **kw)
+    for odd in (99999, 1 << 30, -5):
+        tables = torch.nn.functional.pad(args[3], (0, 2), value=odd)
+        tables[0, 2:] = odd                                       # 12 keys: two pages
+        assert torch.equal(TR.tree_attention(args[0], k[0], v[0], tables, *args[4:], **{**kw, "max_kv": 0}), want)
+    tables = args[3].clone()
+    tables[0, 1] = 1 << 28                                        # times the page size, no id of 32 bits
+    with pytest.raises(IndexError):
+        TR.tree_attention(args[0], k[0], v[0], tables, *args[4:], **kw)
