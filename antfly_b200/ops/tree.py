@@ -291,7 +291,8 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tenso
     ``caches`` holds up to two ``(k, v, slots)`` or ``(k, v, slots, nodes)``: caches of all layers [L, num_blocks, page, ...]
     (or their :class:`antfly_b200.ops.kv_quant.CodecCache`) and the slots [B, nodes] of the nodes, of which only the first
     ``nodes`` were written (a draft model has no rows for its last level).  Row ``slots[b, path[i]]`` is moved to
-    ``slots[b, i]`` in every layer; rows behind the path are left as they were."""
+    ``slots[b, i]`` in every layer; rows behind the path are left as they were.  The slots of all trees differ, and no two
+    of the key and value tensors share memory."""
     B, nodes = tokens.shape if tokens.dim() == 2 else (None, None)
     tokens = _ints("tokens", tokens, B, nodes)
     parents, target = _ints("parents", parents, B, nodes), _ints("target", target, B, nodes)
@@ -308,6 +309,9 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tenso
         if k.dim() < 4 or k.shape[:3] != v.shape[:3] or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("caches must be contiguous [layers, blocks, page, ...]")
         rows.append((k, v, slots, held[0] if held else nodes))
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for r in rows for t in r[:2] if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("keys and values of the caches share memory: their rows would be moved twice")
     if not tokens.is_cuda:
         path, count, following = R.tree_accept(tokens, parents, target, lens)
         for k, v, slots, held in rows:

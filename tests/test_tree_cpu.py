@@ -183,3 +183,16 @@ def test_codec_caches_ask_nothing_of_table_entries_behind_the_last_key():
     tables[0, 1] = 1 << 28                                        # times the page size, no id of 32 bits
     with pytest.raises(IndexError):
         TR.tree_attention(args[0], k[0], v[0], tables, *args[4:], **kw)
+
+
+def test_caches_that_share_memory_are_refused():
+    """Their rows would be moved twice, the second time from where the first move put another node's."""
+    t = i32([[-1, 0, 0, 2, 3]])
+    slots = i32([[0, 1, 2, 3, 4]])
+    k, v = torch.zeros(2, 3, 8, 2, 4), torch.zeros(2, 3, 8, 2, 4)
+    for caches in ([(k, k, slots)], [(k, v, slots), (v, k, slots)], [(k, v, slots), (k, v, slots)],
+                   [(k, v, slots), (k[1:], torch.zeros(1, 3, 8, 2, 4), slots)]):
+        with pytest.raises(ValueError, match="share memory"):
+            TR.tree_accept(t, t, t, caches=caches)
+    both = torch.arange(2 * 2 * 24 * 8, dtype=torch.float32).view(2, 2, 3, 8, 2, 4)      # two halves of one tensor do not
+    TR.tree_accept(t, t, t, caches=[(both[0], both[1], slots)])
