@@ -324,8 +324,8 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tenso
     args = []
     for k, v, slots, held in rows:
         n = k.shape[1] * k.shape[2]
-        args += [k.data_ptr(), v.data_ptr(), k.stride(2) * k.element_size(), v.stride(2) * v.element_size(), k.shape[0], n,
-                 slots.data_ptr(), slots.stride(0), held]
+        row = [math.prod(t.shape[3:]) * t.element_size() for t in (k, v)]   # (a dimension of one has any stride)
+        args += [k.data_ptr(), v.data_ptr(), *row, k.shape[0], n, slots.data_ptr(), slots.stride(0), held]
     args += [0, 0, 0, 0, 0, 0, 0, 0, 0] * (2 - len(rows))
     rc = _lib().afb_tree_accept(tokens.data_ptr(), tokens.stride(0), parents.data_ptr(), parents.stride(0),
                                 target.data_ptr(), target.stride(0), _addr(lens), B, nodes, path.data_ptr(),
