@@ -184,6 +184,8 @@ class LLMEngine:
             raise ValueError("a tree of drafts needs a draft (draft_layers or draft_model)")
         if any(x < 1 for x in branching):
             raise ValueError(f"every level of a tree of drafts has at least one branch, got {branching}")
+        if max(branching) > self.model.cfg.vocab_size:
+            raise ValueError(f"a node has at most the vocabulary's {self.model.cfg.vocab_size} branches, got {branching}")
         if not (getattr(self.model, "tree_drafts", False) and getattr(self.draft, "tree_drafts", False)):
             raise ValueError("trees of drafts are not available for this model (one GPU, no attention sinks or soft caps)")
         levels, parents = [(0, 1)], [-1]

@@ -175,3 +175,13 @@ def test_refusals():
     eng = _engine(draft_layers=1, spec_tree=(2,))
     eng.set_spec_tree(())
     assert eng.spec_tree == ()
+
+
+def test_more_branches_than_tokens_are_refused():
+    few = LlamaModel.random_init(LlamaConfig.tiny(num_hidden_layers=2, vocab_size=64), device="cpu", seed=0)
+    make = lambda **kw: LLMEngine(few, num_blocks=16, page=16, max_batch=2, max_step_tokens=64, use_cuda_graph=False,
+                                  draft_layers=1, **kw)
+    with pytest.raises(ValueError, match="64 branches"):
+        make(spec_tree=(2, 65))
+    sp = SamplingParams(max_tokens=5)
+    assert make(spec_tree=(64, 1)).generate([[7, 8, 9]], sp)[0].token_ids == make().generate([[7, 8, 9]], sp)[0].token_ids
