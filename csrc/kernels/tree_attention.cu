@@ -593,8 +593,8 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 // Tensor memory: three score tiles (the next scores are there before this tile's weights are) and O.
 //
 // e4m3 caches are expanded to fp16, which holds every e4m3 value exactly and takes one conversion instruction per two
-// values (bf16 took five).  Q is brought to fp16 by a power of two per row, to a largest magnitude in [2^14, 2^15): 11 bits
-// for the 8 of bf16, and elements under 2^-28 of their row's largest round to multiples of 2^-39 of it, far below what a sum
+// values (bf16 took five).  Q is brought to fp16 by a power of two per row (2^-114 to 2^100), to a largest magnitude in
+// [2^14, 2^15): 11 bits for the 8 of bf16, and elements under 2^-28 of their row's largest round to multiples of 2^-39 of it, far below what a sum
 // of 32-bit products keeps.  The weights become fp16 as 2^7 times themselves: full 11 bits down to 2^-21 of the maximum.
 // ---------------------------------------------------------------------------------------------------------
 //
@@ -1047,7 +1047,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int o = CH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               // 2^e with top 2^e in [2^14, 2^15); rows of zeros, and rows with an infinity (which stays one), as they are
-              const int ex = top > 0.0f && top < INFINITY ? max(-100, min(100, 14 - ilogbf(top))) : 0;
+              const int ex = top > 0.0f && top < INFINITY ? max(-114, min(100, 14 - ilogbf(top))) : 0;
               const float up = __int_as_float((ex + 127) << 23);
               if (ch == 0) s_power[(seg & 3) * 128 + qr] = static_cast<int8_t>(ex);
               const __half2 h0 = __floats2half2_rn(x0.x * up, x0.y * up), h1 = __floats2half2_rn(x1.x * up, x1.y * up);
@@ -1480,7 +1480,7 @@ int afb_tree_attention(const void* q, long q_stride, const void* k_cache, const 
     return -1;
   }
   // Masked scores are -inf before they are scaled and maxima are taken before it too, so the scale has to be positive; it
-  // stays a normal number after the e4m3 path's powers of two, 2^-100 to 2^100.
+  // stays a normal number after the e4m3 path's powers of two, 2^-100 to 2^114.
   if (!(scale >= 0.99e-7f && scale <= 1.01e4f)) {
     set_last_error("afb_tree_attention: the scale is a positive number from 1e-7 to 1e4, not %g", static_cast<double>(scale));
     return -1;
