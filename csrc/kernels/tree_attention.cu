@@ -1365,18 +1365,28 @@ inline int pick_chunk(long units, int tiles, int slots) {
 }
 
 // Which kernel takes a call.  The tcgen05 one needs pages that TMA can bring, 16-byte rows, no window, and enough work to
-// pay for its start (locating its piece, Q, the first tile: some 6 us, e4m3 a few more) and for its join.  Work is counted
-// in (row, key, KV head) triples at D = 128.  Measured, mma.sync against tcgen05 in us, cold, Hkv = 8, D = 128:
-//   bf16   1 x 8192, 128 rows (8 M): 43 / 49       1 x 32768, 64 rows (17 M): 70 / 70    1 x 8192, 256 rows (17 M): 61 / 43
-//          16 x 500, 64 rows (4 M): 33 / 29        16 x 2000, 20 rows (5 M): 59 / 51     64 x 500, 20 rows (5 M): 59 / 61
-//          64 x 2000, 64 rows (66 M): 234 / 129    4 x 1000, 128 rows (4 M): 31 / 35
-//   e4m3   1 x 8192, 128 rows (8 M): 47 / 64       64 x 500, 64 rows (16 M): 90 / 109    16 x 2000, 48 rows (12 M): 78 / 72
-//          1 x 32768, 128 rows (34 M): 129 / 86    64 x 2000, 20 rows (20 M): 238 / 168
-// Few (sequence, head)s favour mma.sync, whose chunks of 64 keys spread them over more CTAs with less to begin with.
+// pay for its start (locating its piece, Q, the first tile: some 9 us, e4m3 a few more) and for its join.  Work is counted
+// in (row, key, KV head) triples at D = 128.  It also has a fixed cost for every (sequence, head) that a CTA comes to, which
+// up to 64 rows, one row tile of the other kernel, takes several tiles of keys to pay for.  Measured, mma.sync against
+// tcgen05 in us, cold, replayed from a graph, Hkv = 8, D = 128 (* where the rule takes the slower one):
+//   bf16   1 x 8192, 128 rows (8 M): 43 / 49       1 x 32768, 64 rows (17 M): 68 / 68    1 x 8192, 256 rows (17 M): 64 / 43
+//          4 x 1000, 128 rows (4 M): 33 / 35       4 x 4000, 32 rows (4 M): 41 / 39 *    4 x 1000, 256 rows (8 M): 45 / 37
+//          16 x 500, 20 rows (1 M): 27 / 27        16 x 500, 64 rows (4 M): 33 / 29      16 x 2000, 20 rows (5 M): 61 / 51
+//          64 x 250, 64 rows (8 M): 51 / 64        64 x 250, 128 rows (16 M): 90 / 77    64 x 500, 20 rows (5 M): 59 / 61 *
+//          64 x 1000, 20 rows (10 M): 102 / 80     64 x 2000, 64 rows (66 M): 246 / 131  200 x 500, 64 rows (51 M): 209 / 172
+//   e4m3   1 x 8192, 128 rows (8 M): 47 / 64       1 x 32768, 64 rows (17 M): 76 / 84    1 x 8192, 256 rows (17 M): 76 / 61
+//          4 x 4000, 64 rows (8 M): 45 / 53        4 x 4000, 128 rows (16 M): 78 / 56    16 x 500, 128 rows (8 M): 49 / 49
+//          16 x 2000, 32 rows (8 M): 72 / 76       16 x 2000, 48 rows (12 M): 80 / 75 *  64 x 250, 128 rows (16 M): 103 / 113 *
+//          1 x 65536, 20 rows (10 M): 113 / 107    4 x 8192, 64 rows (17 M): 78 / 78     8 x 8192, 20 rows (10 M): 125 / 110
+//          64 x 500, 64 rows (16 M): 90 / 113      64 x 500, 128 rows (33 M): 160 / 127  64 x 1000, 32 rows (16 M): 129 / 127
+//          64 x 2000, 20 rows (20 M): 242 / 182    200 x 500, 64 rows (51 M): 240 / 291  200 x 500, 128 rows (102 M): 453 / 307
+// Few (sequence, head)s favour mma.sync, whose chunks of 64 keys spread them over more CTAs with less to begin with.  On
+// e4m3 both times go by the keys alone up to 64 rows: mma.sync has its one row tile, tcgen05 its expansion.
 inline bool use_tc(long units, int rows, int D, int kv8, int window, int page, int max_kv) {
   if (window > 0 || D > 128 || (kv8 && D % 16) || page % 8 || rows <= 16) return false;
   const double work = static_cast<double>(units) * rows * max_kv * D / 128;
-  return work >= (kv8 ? 16e6 : units < 32 ? 14e6 : 5e6);
+  if (kv8) return rows > 64 ? work >= 16e6 : max_kv >= 1000 && work >= 4e5 * rows;
+  return (rows > 64 || max_kv >= 500) && work >= (units < 32 ? 14e6 : units < 128 ? 5e6 : 2e6);
 }
 
 template <int DP, bool KV8>
