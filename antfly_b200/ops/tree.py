@@ -180,7 +180,10 @@ def tree_attention(q, k_cache, v_cache, block_tables, q_starts, q_lens, kv_lens,
     :func:`tree_plan`, or any other; a batch dimension expanded from 1 serves one tree shape for all.  A row that sees
     no key comes back as zeros.  ``window`` > 0 (needs ``depths``) keeps the keys at positions > the row's position -
     ``window``, a node's position being the tree's first key plus its depth.  ``scale`` (default 1 / sqrt(D)) is a positive
-    number from 1e-7 to 1e4.
+    number from 1e-7 to 1e4; scaled scores lie below 2^30 in magnitude.
+
+    Scores, their maxima, the sums of the weights and the output are kept in 32 bits.  For the product with V the GPU rounds
+    each weight once to 16 bits (bf16; fp16 over e4m3 caches with many rows), and the output to bf16 in the end.
 
     ``max_q_len`` bounds ``q_lens`` and ``max_kv`` (0: what the block table can hold) bounds ``kv_lens``; both size the
     launch, and a length past them is reported through the status word.  A window of ``max_kv`` keys or more is none.

@@ -175,7 +175,10 @@ class LLMEngine:
     def set_spec_tree(self, branching: Sequence[int]) -> None:
         """Drafts of a round form a tree: every node of level d has the draft model's ``branching[d]`` most likely next
         tokens as children ((4, 2, 1): 1 + 4 + 8 + 8 nodes with the last accepted token).  The target checks all nodes in
-        one pass and the longest path it agrees with is kept.  () goes back to chains of ``spec_k``."""
+        one pass and the longest path it agrees with is kept.  () goes back to chains of ``spec_k``.  A round whose tree
+        does not fit behind a sequence or into the pool is a chain (there a request's ``speculative_k`` counts), and one
+        without room for that a plain step.  Over a cache kept as int8, int4, polar4 or turbo3 every pass of a round expands
+        its contexts to bf16, where a chain's drafting reads the codes."""
         branching = tuple(int(x) for x in branching)
         if not branching:
             self.spec_tree, self._tree = (), None

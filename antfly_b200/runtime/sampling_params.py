@@ -20,7 +20,8 @@ class SamplingParams:
     seed: Optional[int] = None
     cache_compaction_ratio: Optional[float] = None  # in (0, 1): compact the KV cache to this fraction after prefill
     grammar: Optional[object] = None  # antfly_b200.runtime.grammar.JsonGrammar: constrains every sampled token
-    speculative_k: Optional[int] = None  # draft tokens per speculative round (1..16); None: the engine's default
+    speculative_k: Optional[int] = None  # draft tokens of a chain per round (1..16); None: the engine's default.  Where the
+    # engine drafts trees, only rounds that have no room for its tree are chains
 
     @property
     def greedy(self) -> bool:

@@ -264,8 +264,8 @@ __device__ __forceinline__ uint64_t tree_bits(const TreeAttnParams& p, const Tre
 // head-in-group) rows of one KV head against one chunk of its keys, on mma.sync with a three-stage cp.async ring.  Four
 // warps: WR of them own 16 rows each, and 4 / WR groups share the 64 keys of a tile.  Bound by memory up to some 16 rows (64 x
 // 2000 keys, 12 rows, 32 / 8 heads of 128: 174 us cold, 3.0 TB/s), by the four warps' instructions above.  One request of 8192
-// keys and a tree of 26: 37 us; 12 x 5000 keys, a window of 1024, 256-wide heads, pages of 24: 45 us, where the 229 KiB of the
-// ring and Q leave one CTA of four warps on an SM.
+// keys and a tree of 26: 37 us; 12 x 5000 keys, a window of 1024, 256-wide heads, pages of 24: 45 us, where the 208 KiB of the
+// ring and Q leave one CTA of four warps on an SM.  Weights are rounded to bf16 for the product with V, their sum is not.
 template <int DP, int WR, bool KV8>
 struct MmaShape {
   static constexpr int kRow = DP * (KV8 ? 1 : 2);
@@ -574,7 +574,8 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 // Work split.  The batch's tiles (sequence, block of KV heads, key tile) form one line, cut into as many equal pieces as the
 // GPU has groups of `heads x row_tiles` CTAs; the CTAs of a group take one KV head of the block and one row tile each
 // over the same piece.  So the heads of a token, which lie next to one another in a page, are read at about the same time
-// (DRAM rows are opened once), and K and V come from L2 for all row tiles but one.  A piece ends anywhere in a sequence: a CTA has at most two segments that are not a whole (sequence,
+// (DRAM rows are opened once), and K and V come from L2 for all row tiles but one.
+// A piece ends anywhere in a sequence: a CTA has at most two segments that are not a whole (sequence,
 // head), stores those in 32 bits with their log-sum, and a second kernel joins them.  Sequences of any mix of lengths keep
 // every SM busy until the end, and the partial rows take 2 x 128 rows per CTA whatever the lengths.
 //
@@ -582,7 +583,10 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 //   0-7  softmax: two threads per row (a row is a lane of tensor memory, which two warps may read), 64 keys each, who tell
 //        each other their maxima.  A thread reads its scores into registers and writes the weights as packed 16-bit
 //        numbers over scores that both have read.  O is rescaled only when a row's maximum grew by more than 2^8 over the
-//        one in use: weights then reach 2^8 at most, which neither their relative rounding nor the 32-bit sums mind.
+//        one in use: weights then reach 2^8 at most, which the 32-bit sums do not mind.  bf16 caches take bf16 weights
+//        (A and B of a product have one type): 2^-9 of a weight on average, of the largest too, which would be exactly 1
+//        under its own maximum.  Against 64 bits the output is off by 2.3e-3 of its spread, 1.7e-3 of which is its own
+//        rounding to bf16; the mma.sync kernel, whose maximum never lags, by 1.8e-3, and fp16 weights by 1.7e-3.
 //   8-11 Q to shared memory, and what TMA cannot do: e4m3 tiles are expanded, and values that are no numbers are taken out
 //        of V tiles with masked keys (0 times such a value is no zero), see `careful` below.
 //   12   one thread issues S = Q K^T (both K-major) and O += P V (P from tensor memory, V as it lies: MN-major) as their
@@ -594,18 +598,21 @@ __global__ void __launch_bounds__(128) tree_attn_mma_kernel(const TreeAttnParams
 //
 // e4m3 caches are expanded to fp16, which holds every e4m3 value exactly and takes one conversion instruction per two
 // values (bf16 took five).  Q is brought to fp16 by a power of two per row (2^-114 to 2^100), to a largest magnitude in
-// [2^14, 2^15): 11 bits for the 8 of bf16, and elements under 2^-28 of their row's largest round to multiples of 2^-39 of it, far below what a sum
-// of 32-bit products keeps.  The weights become fp16 as 2^7 times themselves: full 11 bits down to 2^-21 of the maximum.
+// [2^14, 2^15): 11 bits for the 8 of bf16, and elements under 2^-28 of their row's largest round to multiples of 2^-39 of
+// it, far below what a sum of 32-bit products keeps.  The weights become fp16 as 2^7 times themselves: full 11 bits down to
+// 2^-21 of the maximum.
 // ---------------------------------------------------------------------------------------------------------
 //
 // Measured (B200, in the order of a program's calls): 64 sequences of up to 2048 keys, trees of up to 16, 32 / 8 heads of 128:
-// 96 us (3.7 TB/s); 16 x 8192 keys, trees of 21, 64 / 8 heads: 207 us (2.7 TB/s, 435 TFLOP/s); one of 131072 keys, a tree of
-// 64 (two row tiles): 210 us (2.6 TB/s, 656 TFLOP/s); 32 x 4096 keys of e4m3, trees of 13: 146 us.  bf16 with one row tile is
-// bound by memory in its steady state (a 64 KiB pair of tiles per SM and 1.76 us: 5.2 TB/s over the 148 SMs, as the decode
-// kernel's cp.async ring gets) and by some 6 us to its first scores; e4m3 by the expansion (1500 cycles of four warps a
-// tile, two tiles a step).  What was tried and lost: cp.async instead of TMA (105 us in the first case), one softmax group
-// with all 128 scores in registers (124 us: it spills, and spills miss an L1 of 28 KiB), two groups on alternate tiles
-// with an O each (141 us: no room for a third score tile, so each waits for its own product).
+// 98 us (3.6 TB/s); 16 x 8192 keys, trees of 21, 64 / 8 heads: 211 us (2.6 TB/s, 428 TFLOP/s); one of 131072 keys, a tree of
+// 64 (two row tiles): 212 us (2.5 TB/s, 646 TFLOP/s); 32 x 4096 keys of e4m3, trees of 13: 156 us.  One level of a tree, 8 rows
+// of 21 nodes over 64 x 2048 keys: 113 us, e4m3 186 us (4 rows, on mma.sync: 162 and 210).  bf16 with one row tile is bound by
+// memory in its steady state (a 64 KiB pair of tiles per SM and 1.76 us: 5.5 TB/s over the 148 SMs), by 7 to 9 us to its
+// first weights and by the ends of its segments, some 2 us each; e4m3 by the expansion (1500 cycles of four warps a tile, two
+// tiles a step).  Both 64-wide kernels spill 16 to 32 bytes, the 128-wide ones nothing.
+// What was tried and lost, in the first case: cp.async instead of TMA (105 us), one softmax group with all 128 scores in
+// registers (124 us: it spills, and spills miss an L1 of 28 KiB), two groups on alternate tiles with an O each (141 us: no
+// room for a third score tile, so each waits for its own product).
 constexpr int kTcKeys = 128;
 constexpr int kTcThreads = 480;
 constexpr int kMaxTcNodes = 256;

@@ -19,8 +19,8 @@ constexpr int kMaxTreeWords = kMaxTreeNodes / 32;
 //   table[b][j] = blocks[o_b + j] for j < n_b, 0 behind;   slot of row s_b + i = table[b][(kv_b + i) / page] * page
 //   + (kv_b + i) % page;   position = kv_b + i, or with depths kv_b - (tree_b - q_b) + depth of node tree_b - q_b + i.
 // A CTA owns `per_cta` sequences (and one of gridDim.y slices of their rows): it sums the lengths in front of them
-// itself, so there is one launch and no pass over the lengths before it.  3.4 us in a graph for 64 sequences, 11.5 us with
-// the plan of 512 trees of 64 nodes and tables of 4160 entries (14.5 MB): latency, the tables' stores at 1.3 TB/s.
+// itself, so there is one launch and no pass over the lengths before it.  4.2 us in a graph for 64 sequences, 10.3 us with
+// the plan of 512 trees of 64 nodes and tables of 4160 entries (14.5 MB): latency, the tables' stores at 1.4 TB/s.
 // ---------------------------------------------------------------------------------------------------------
 struct StepMapsParams {
   const int* kv_before;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(256) tree_plan_kernel(const int* parents, long
 // target's choice at the current node; path[i] is the i-th node on it.  Links point to earlier nodes, so path[i] >= i and
 // the path ascends: a thread that owns one 16-byte column of the rows may move row path[i] to row i for i = 1, 2, ...
 // in place, several loads ahead of their stores, without ever overwriting a row that is still to be read.  Every CTA walks
-// its tree itself (a warp, a ballot per step), which takes less than a second launch.  3.4 us in a graph for one tree; 12 us for
+// its tree itself (a warp, a ballot per step), which takes less than a second launch.  4.8 us in a graph for one tree; 12 us for
 // 64 trees of 64 nodes over 32 layers of 2 KiB rows (about 50 MB moved, 4.2 TB/s).
 // ---------------------------------------------------------------------------------------------------------
 struct AcceptCache {
