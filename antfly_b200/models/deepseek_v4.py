@@ -305,7 +305,10 @@ class DeepseekV4Model:
         return DeepseekV4State()
 
     def _lin(self, x: torch.Tensor, wt: torch.Tensor) -> torch.Tensor:
-        return Dn.gemm_bf16(x.to(self.dtype).contiguous(), wt, out_dtype=torch.float32).float()
+        x, odd = x.to(self.dtype).contiguous(), -x.shape[1] % 8
+        if odd and x.is_cuda:                        # the GEMM takes rows of a multiple of 16 bytes
+            x, wt = (torch.nn.functional.pad(t, (0, odd)) for t in (x, wt))
+        return Dn.gemm_bf16(x, wt, out_dtype=torch.float32).float()
 
     # -- compressed pools --------------------------------------------------------------------------------------
     def _update_pool(self, st: Optional[CompressorState], h: torch.Tensor, prefix: str, rate: int, row_dim: int,
