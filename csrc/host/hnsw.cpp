@@ -57,6 +57,8 @@ struct Hnsw {
   std::vector<uint64_t> ids;
   std::vector<std::string> meta;
   std::vector<uint32_t> free_slots;
+  std::vector<uint32_t> in0;             // edges into each slot on layer 0
+  bool cut_off = false;                  // some node lost its last edge of those since the last reconnect
   std::unordered_map<uint64_t, uint32_t> slot_of;
   uint32_t entry = kNone;
   int max_level = -1;
@@ -173,6 +175,11 @@ struct Hnsw {
 
   void set_links(uint32_t s, int l, const std::vector<uint32_t>& list) {
     uint32_t* nb = nbrs(s, l);
+    if (l == 0) {
+      for (uint32_t t : list) ++in0[t];
+      for (uint32_t i = 1; i <= nb[0]; ++i)
+        if (--in0[nb[i]] == 0) cut_off = true;
+    }
     nb[0] = static_cast<uint32_t>(list.size());
     for (size_t i = 0; i < list.size(); ++i) nb[1 + i] = list[i];
   }
@@ -184,6 +191,7 @@ struct Hnsw {
       if (nb[i] == t) return;
     if (static_cast<int>(nb[0]) < cap(l)) {
       nb[++nb[0]] = t;
+      if (l == 0) ++in0[t];
       return;
     }
     std::vector<Cand> cands;
@@ -215,6 +223,7 @@ struct Hnsw {
     up.emplace_back();
     vecs.resize(static_cast<size_t>(s + 1) * dim);
     links0.resize(static_cast<size_t>(s + 1) * (M0 + 1), 0);
+    in0.push_back(0);
     return s;
   }
 
@@ -300,12 +309,12 @@ struct Hnsw {
     }
     for (uint32_t s : gone_list) {
       if (level[s] < 0) continue;
+      set_links(s, 0, {});
       slot_of.erase(ids[s]);
       level[s] = -1;
       up[s].clear();
       up[s].shrink_to_fit();
       meta[s].clear();
-      links0[static_cast<size_t>(s) * (M0 + 1)] = 0;
       free_slots.push_back(s);
       --active;
     }
@@ -318,6 +327,63 @@ struct Hnsw {
           entry = s;
         }
     }
+  }
+
+  // Gives every node that layer 0 does not lead to from the entry point an edge from the nearest node that it does lead
+  // to: pruned lists and removed nodes may leave a node, or a few that only point at one another, out of every search.
+  // A full list gives up its farthest neighbour that others point at, too; what this cuts off, the next pass finds.
+  void reconnect() {
+    cut_off = false;
+    for (int pass = 0; pass < 8 && entry != kNone && reconnect_pass(); ++pass) {}
+  }
+  bool reconnect_pass() {                // whether an edge was given up
+    bool gave_up = false;
+    const uint32_t n = static_cast<uint32_t>(level.size());
+    std::vector<uint8_t> reached(n, 0);
+    std::vector<uint32_t> stack;
+    const auto spread = [&](uint32_t from) {
+      reached[from] = 1;
+      stack.push_back(from);
+      while (!stack.empty()) {
+        const uint32_t* nb = nbrs(stack.back(), 0);
+        stack.pop_back();
+        for (uint32_t i = 1; i <= nb[0]; ++i)
+          if (!reached[nb[i]]) {
+            reached[nb[i]] = 1;
+            stack.push_back(nb[i]);
+          }
+      }
+    };
+    spread(entry);
+    if (build_seen.size() < n) build_seen.resize(n + n / 2 + 64, 0);
+    std::vector<Cand> found;
+    for (uint32_t s = 0; s < n; ++s) {
+      if (level[s] < 0 || reached[s]) continue;
+      search_layer(vec(s), entry, efc, 0, build_seen, [&](uint32_t x) { return x != s; }, found);
+      bool done = false;
+      for (size_t i = 0; i < found.size() && !done; ++i)
+        if (static_cast<int>(nbrs(found[i].s, 0)[0]) < M0) {
+          connect(found[i].s, s, 0);
+          done = true;
+        }
+      for (size_t i = 0; i < found.size() && !done; ++i) {
+        uint32_t* nb = nbrs(found[i].s, 0);
+        uint32_t worst = 0;
+        float far = -std::numeric_limits<float>::infinity();
+        for (uint32_t j = 1; j <= nb[0]; ++j) {
+          const float d = dist(vec(found[i].s), vec(nb[j]));
+          if (in0[nb[j]] > 1 && d > far) { far = d; worst = j; }
+        }
+        if (worst == 0) continue;
+        --in0[nb[worst]];
+        gave_up = true;
+        nb[worst] = s;
+        ++in0[s];
+        done = true;
+      }
+      if (done) spread(s);
+    }
+    return gave_up;
   }
 };
 
@@ -360,6 +426,7 @@ int afb_hnsw_insert(void* p, const uint64_t* ids, const float* vecs, long n, con
     const long len = meta_blob && meta_offsets ? meta_offsets[i + 1] - meta_offsets[i] : 0;
     h->insert_one(ids[i], vecs + static_cast<size_t>(i) * h->dim, md, len, levels ? levels[i] : -1);
   }
+  if (h->cut_off) h->reconnect();
   return 0;
 }
 
@@ -447,6 +514,7 @@ long afb_hnsw_delete(void* p, const uint64_t* ids, long n) {
     if (it != h->slot_of.end() && std::find(gone.begin(), gone.end(), it->second) == gone.end()) gone.push_back(it->second);
   }
   h->remove_slots(gone);
+  h->reconnect();
   return static_cast<long>(gone.size());
 }
 
@@ -461,6 +529,7 @@ long afb_hnsw_delete_by_metadata(void* p, const uint8_t* key, int len) {
         std::memcmp(h->meta[s].data(), key, static_cast<size_t>(len)) == 0)
       gone.push_back(s);
   h->remove_slots(gone);
+  h->reconnect();
   return static_cast<long>(gone.size());
 }
 
@@ -616,6 +685,10 @@ void* afb_hnsw_load(const char* path, uint64_t seed) {
     delete h;
     return nullptr;
   }
+  h->in0.assign(n, 0);
+  for (uint64_t s = 0; s < n; ++s)
+    if (h->level[s] >= 0)
+      for (uint32_t i = 1; i <= h->nbrs(static_cast<uint32_t>(s), 0)[0]; ++i) ++h->in0[h->nbrs(static_cast<uint32_t>(s), 0)[i]];
   return h;
 }
 

@@ -176,3 +176,23 @@ def test_graph_index_as_a_tables_dense_index():
     assert hits[0].id == "k17"
     t.delete("k17")
     assert all(h.id != "k17" for h in t.query(TableQuery(embedding=emb[17], limit=3)))
+
+
+def test_every_stored_vector_stays_reachable():
+    """Four links a node, batches of inserts and deletes: each live vector is the nearest to itself, in a search wide enough
+    for all of them."""
+    for seed in range(150):
+        rng = np.random.default_rng(seed)
+        idx, live = HNSWIndex(8, "l2_squared", neighbors=4, ef_construction=20, ef_search=20, seed=seed), {}
+        for _ in range(5):
+            ids = rng.integers(0, 60, rng.integers(1, 25)).tolist()
+            vecs = rng.standard_normal((len(ids), 8)).astype(np.float32)
+            idx.batch_insert(ids, torch.from_numpy(vecs))
+            live.update(zip(ids, vecs))
+            for gone in ([], [i for i in live if rng.random() < 0.3]):
+                idx.delete(gone)
+                for i in gone:
+                    del live[i]
+                if live:
+                    found = idx.search(torch.from_numpy(np.stack(list(live.values()))), 1, ef=64).ids.flatten().tolist()
+                    assert found == list(live) and idx.check() == 0
