@@ -305,16 +305,18 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tenso
         lens = _ints("lens", lens, B)
     if len(caches) > 2:
         raise ValueError("at most two caches")
-    rows = []
+    rows, spans = [], []
     for k, v, slots, *held in caches:
         k, v = getattr(k, "data", k), getattr(v, "data", v)
         slots = _ints("slots", slots, B, nodes)
         if k.dim() < 4 or k.shape[:3] != v.shape[:3] or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("caches must be contiguous [layers, blocks, page, ...]")
         rows.append((k, v, slots, held[0] if held else nodes))
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for r in rows for t in r[:2] if t.numel())
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise ValueError("keys and values of the caches share memory: their rows would be moved twice")
+        spans += (k.data_ptr(), k.nbytes), (v.data_ptr(), v.nbytes)
+    for i, (a, n) in enumerate(spans):
+        for b, m in spans[:i]:
+            if a < b + m and b < a + n:
+                raise ValueError("keys and values of the caches share memory: their rows would be moved twice")
     if not tokens.is_cuda:
         path, count, following = R.tree_accept(tokens, parents, target, lens)
         for k, v, slots, held in rows:
@@ -325,10 +327,11 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tenso
     path, count, following = buf.split_with_sizes([B * nodes, B, B])
     path = path.view(B, nodes)
     args = []
-    for k, v, slots, held in rows:
-        n = k.shape[1] * k.shape[2]
-        row = [math.prod(t.shape[3:]) * t.element_size() for t in (k, v)]   # (a dimension of one has any stride)
-        args += [k.data_ptr(), v.data_ptr(), *row, k.shape[0], n, slots.data_ptr(), slots.stride(0), held]
+    for i, (k, _, slots, held) in enumerate(rows):
+        (k_at, k_bytes), (v_at, v_bytes) = spans[2 * i:2 * i + 2]
+        layers, blocks, page = k.shape[:3]
+        n = max(layers * blocks * page, 1)                   # (row sizes not from strides: a dimension of one has any)
+        args += [k_at, v_at, k_bytes // n, v_bytes // n, layers, blocks * page, slots.data_ptr(), slots.stride(0), held]
     args += [0, 0, 0, 0, 0, 0, 0, 0, 0] * (2 - len(rows))
     rc = _lib().afb_tree_accept(tokens.data_ptr(), tokens.stride(0), parents.data_ptr(), parents.stride(0),
                                 target.data_ptr(), target.stride(0), _addr(lens), B, nodes, path.data_ptr(),
